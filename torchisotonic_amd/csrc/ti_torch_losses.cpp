@@ -58,6 +58,14 @@ void once(const char* what) {
 // Whether a backward may follow (asked outside the autograd node's forward, which runs untracked).
 bool tracked(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 
+// A saved tensor as the kernels take it. (What comes back is what saved-tensor hooks made of it: a copy, maybe in
+// another layout, so that nothing of the layout it was saved in holds.)
+at::Tensor saved_as(const at::Tensor& t, int64_t numel, at::ScalarType type, const at::Device& device, const char* what) {
+  TORCH_CHECK(t.defined() && t.numel() == numel && t.scalar_type() == type && t.device() == device, "torchisotonic_amd.",
+              what, " backward: a saved tensor came back with another size, type or device");
+  return t.contiguous();
+}
+
 at::Tensor workspace(size_t bytes, const at::Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
@@ -133,8 +141,7 @@ struct LogprobsFn : public torch::autograd::Function<LogprobsFn> {
     Logprobs out = logprobs_of(logits, targets, temperature, ignore_index, entropy, true);
     ctx->set_materialize_grads(false);  // (an output that no gradient comes for costs no launch)
     ctx->save_for_backward({out.where.logits, targets, out.stats, out.entropy});
-    ctx->saved_data["p"] =
-        c10::List<int64_t>({ignore_index, out.where.inner, out.where.outer_stride, out.where.row_stride});
+    ctx->saved_data["i"] = ignore_index;
     ctx->saved_data["t"] = temperature;
     if (entropy) return {out.logp, out.entropy};
     return {out.logp};
@@ -147,15 +154,26 @@ struct LogprobsFn : public torch::autograd::Function<LogprobsFn> {
     const at::Tensor ge = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
     if (!g.defined() && !ge.defined()) return none;
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &logits = saved[0], &t = saved[1], &stats = saved[2], &h = saved[3];
-    const c10::List<int64_t> p = ctx->saved_data["p"].toIntList();
-    const c10::DeviceGuard guard(logits.device());
+    const at::Tensor &logits = saved[0], &up = g.defined() ? g : ge;
+    const c10::DeviceGuard guard(up.device());
+    const int64_t rows = up.numel();
+    TORCH_CHECK(logits.device() == up.device() && logits.dim() == up.dim() + 1 &&
+                    logits.sizes().slice(0, up.dim()) == up.sizes() &&
+                    (logits.scalar_type() == at::kDouble) == (up.scalar_type() == at::kDouble),
+                "torchisotonic_amd.token_logprobs backward: the saved logits came back with another size, type or device");
     at::Tensor out = at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
-    check(ti_logprobs_bwd(ptr(logits), t.data_ptr<int64_t>(), ptr(stats), ptr(h), ptr(g), ptr(ge), ptr(out), t.numel(),
-                          logits.size(-1), p.get(1), p.get(2), p.get(3), p.get(0), ctx->saved_data["t"].toDouble(),
+    none[0] = out;
+    if (rows == 0) return none;
+    const at::Tensor t = saved_as(saved[1], rows, at::kLong, up.device(), "token_logprobs");
+    const at::Tensor stats = saved_as(saved[2], 2 * rows, up.scalar_type(), up.device(), "token_logprobs");
+    const at::Tensor h = ge.defined() ? saved_as(saved[3], rows, up.scalar_type(), up.device(), "token_logprobs") : at::Tensor();
+    std::optional<Rows> r = rows_of(logits);
+    const Rows where = r.has_value() ? *r : *rows_of(logits.contiguous());
+    check(ti_logprobs_bwd(ptr(where.logits), t.data_ptr<int64_t>(), ptr(stats), ptr(h), ptr(g), ptr(ge), ptr(out), rows,
+                          logits.size(-1), where.inner, where.outer_stride, where.row_stride,
+                          ctx->saved_data["i"].toInt(), ctx->saved_data["t"].toDouble(),
                           dtype_code(logits, "token_logprobs"), stream_of(logits)),
           "token_logprobs backward");
-    none[0] = out;
     return none;
   }
 };
@@ -259,14 +277,19 @@ struct PreferenceFn : public torch::autograd::Function<PreferenceFn> {
     variable_list none(9);
     if (!grads[0].defined()) return none;
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &slopes = saved[0], &offsets = saved[1], &mask = saved[2];
     const std::vector<int64_t> p = ctx->saved_data["p"].toIntVector();
     const at::Tensor g = grads[0].contiguous();
-    const c10::DeviceGuard guard(slopes.device());
-    at::Tensor out = at::empty(at::IntArrayRef(p).slice(4), slopes.options());
+    const c10::DeviceGuard guard(g.device());
+    at::Tensor out = at::empty(at::IntArrayRef(p).slice(4), g.options());
     if (p[1] == 0) {
       out.zero_();
     } else {
+      const at::Tensor slopes = saved_as(saved[0], p[1], g.scalar_type(), g.device(), "preference_loss");
+      const at::Tensor offsets = saved[1].defined()
+                                     ? saved_as(saved[1], p[1] + 1, at::kLong, g.device(), "preference_loss")
+                                     : at::Tensor();
+      const at::Tensor mask =
+          saved[2].defined() ? saved_as(saved[2], p[0], at::kBool, g.device(), "preference_loss") : at::Tensor();
       check(ti_preference_bwd(static_cast<const uint8_t*>(ptr(mask)), static_cast<const int64_t*>(ptr(offsets)), p[0],
                               p[1], p[2], ptr(slopes), ptr(g), static_cast<int>(p[3]), ptr(out),
                               dtype_code(slopes, "preference_loss"), stream_of(slopes)),
@@ -295,9 +318,21 @@ struct PolicyCall {
   double clip_low, clip_high, kl_coef;
   int64_t reduction;
 
-  void operator()(const at::Tensor& loss, const at::Tensor& more, const at::Tensor& grad) const {
-    const Sequences s =
-        sequences_of(logps, offsets.defined() ? std::optional<at::Tensor>(offsets) : std::nullopt, "policy_loss");
+  // The sequences, once every tensor is checked.
+  Sequences checked() const {
+    auto some = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+    const Sequences s = sequences_of(logps, some(offsets), "policy_loss");
+    check_like(logps, old, logps.scalar_type(), "old_logps", "policy_loss");
+    check_like(logps, some(ref), logps.scalar_type(), "reference_logps", "policy_loss");
+    check_like(logps, some(mask), at::kBool, "mask", "policy_loss");
+    TORCH_CHECK((advantages.sizes() == logps.sizes() || (advantages.dim() == 1 && advantages.numel() == s.count)) &&
+                    advantages.device() == logps.device() && advantages.scalar_type() == logps.scalar_type() &&
+                    advantages.is_contiguous(),
+                "torchisotonic_amd.policy_loss: advantages must be one a token or one a sequence, and match logps");
+    return s;
+  }
+
+  void operator()(const Sequences& s, const at::Tensor& loss, const at::Tensor& more, const at::Tensor& grad) const {
     const bool each = advantages.sizes() == logps.sizes();
     size_t bytes = 0;
     check(ti_policy_workspace(s.total, s.count, &bytes), "policy_loss");
@@ -319,17 +354,10 @@ struct PolicyFn : public torch::autograd::Function<PolicyFn> {
                                const at::Tensor& advantages, const std::optional<at::Tensor>& ref,
                                const std::optional<at::Tensor>& offsets, const std::optional<at::Tensor>& mask,
                                double clip_low, double clip_high, double kl_coef, int64_t reduction, bool want) {
-    const Sequences s = sequences_of(logps, offsets, "policy_loss");
-    check_like(logps, old, logps.scalar_type(), "old_logps", "policy_loss");
-    check_like(logps, ref, logps.scalar_type(), "reference_logps", "policy_loss");
-    check_like(logps, mask, at::kBool, "mask", "policy_loss");
-    TORCH_CHECK((advantages.sizes() == logps.sizes() || (advantages.dim() == 1 && advantages.numel() == s.count)) &&
-                    advantages.device() == logps.device() && advantages.scalar_type() == logps.scalar_type() &&
-                    advantages.is_contiguous(),
-                "torchisotonic_amd.policy_loss: advantages must be one a token or one a sequence, and match logps");
-    const c10::DeviceGuard guard(logps.device());
     const PolicyCall call{logps, old, advantages, ref.value_or(at::Tensor()), mask.value_or(at::Tensor()),
                           offsets.value_or(at::Tensor()), clip_low, clip_high, kl_coef, reduction};
+    const Sequences s = call.checked();
+    const c10::DeviceGuard guard(logps.device());
     // (the loss a tensor of its own: a view made here could not be changed in place by the caller)
     at::Tensor loss, more, grad;
     if (s.count == 0) {
@@ -340,12 +368,13 @@ struct PolicyFn : public torch::autograd::Function<PolicyFn> {
       loss = at::empty({}, logps.options());
       more = at::empty({2}, logps.options());
       if (want) grad = at::empty_like(logps);
-      call(loss, more, grad);
+      call(s, loss, more, grad);
     }
     if (want) {
       ctx->save_for_backward({logps, old, advantages, call.ref, call.mask, call.offsets});
       ctx->saved_data["grad"] = grad;
-      ctx->saved_data["p"] = c10::List<double>({clip_low, clip_high, kl_coef, static_cast<double>(reduction)});
+      ctx->saved_data["p"] = c10::List<double>(
+          {clip_low, clip_high, kl_coef, static_cast<double>(reduction), static_cast<double>(s.total)});
     }
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({more});
@@ -363,14 +392,17 @@ struct PolicyFn : public torch::autograd::Function<PolicyFn> {
       grad = held->second.toTensor();
       ctx->saved_data.erase(held);
     } else {
-      const variable_list t = ctx->get_saved_variables();
+      variable_list t = ctx->get_saved_variables();
+      for (at::Tensor& saved : t)
+        if (saved.defined()) saved = saved_as(saved, saved.numel(), saved.scalar_type(), g.device(), "policy_loss");
       const c10::List<double> p = ctx->saved_data["p"].toDoubleList();
+      TORCH_CHECK(t[0].scalar_type() == g.scalar_type() && t[0].numel() == static_cast<int64_t>(p.get(4)),
+                  "torchisotonic_amd.policy_loss backward: a saved tensor came back with another size or type");
+      const PolicyCall call{t[0], t[1], t[2], t[3], t[4], t[5], p.get(0), p.get(1), p.get(2), static_cast<int64_t>(p.get(3))};
+      const Sequences s = call.checked();
       grad = at::empty_like(t[0]);
-      if (sequences_of(t[0], t[5].defined() ? std::optional<at::Tensor>(t[5]) : std::nullopt, "policy_loss").count == 0)
-        grad.zero_();
-      else
-        PolicyCall{t[0], t[1], t[2], t[3], t[4], t[5], p.get(0), p.get(1), p.get(2), static_cast<int64_t>(p.get(3))}(
-            at::empty({}, g.options()), at::empty({2}, g.options()), grad);
+      if (s.count == 0) grad.zero_();
+      else call(s, at::empty({}, g.options()), at::empty({2}, g.options()), grad);
     }
     check(ti_policy_bwd(ptr(grad), grad.numel(), ptr(g), dtype_code(g, "policy_loss"), stream_of(g)),
           "policy_loss backward");
