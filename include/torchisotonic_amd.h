@@ -447,7 +447,7 @@ int ti_pool(const void* keys, const int64_t* order, const void* y, const void* w
  *   logp     [rows] log softmax(logits / temperature) at the target, float32 (float64 for TI_F64).
  *   entropy  [rows] -sum p log p of that softmax, or NULL; the type of logp.
  *   stats    [2, rows] for ti_logprobs_bwd: each row's largest logit, and the sum of its
- *            exp((z - largest) / temperature), up to a factor of a rounding; the type of logp. NULL
+ *            exp((z - largest) / temperature), up to a factor of sqrt(2); the type of logp. NULL
  *            where no backward follows.
  *   workspace / workspace_bytes: at least ti_logprobs_workspace() bytes, 256-byte aligned (0 but for
  *            few long rows, which several workgroups share).

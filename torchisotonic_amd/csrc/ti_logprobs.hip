@@ -45,18 +45,30 @@ __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b)
 __device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
-// Beyond `huge` a logit times log2(e) / T is near the end of the range; `lowest` stands in for an exponent of
-// -inf, finite also times a sum.
+// Up to `near` the rounding of a logit times log2(e) / T is at most half a binade; `lowest` stands in for an
+// exponent of -inf: its power is zero, as that of every exponent below it is.
 template <typename A>
 struct Limits;
 template <>
 struct Limits<float> {
-  static constexpr float huge = 1.0e37f, lowest = -1.0e30f;
+  static constexpr float near = 0x1p24f, lowest = -1.0e4f, largest = 3.402823466e38f;
 };
 template <>
 struct Limits<double> {
-  static constexpr double huge = 1.0e307, lowest = -1.0e300;
+  static constexpr double near = 0x1p53, lowest = -1.0e4, largest = 1.7976931348623157e308;
 };
+
+// log2(e) / T and 1 / T in the type of the sums; the largest finite value where T is too small for them (what is
+// not a row's largest logit has probability zero long before).
+template <typename A>
+__device__ __forceinline__ A per_temperature(double x, double temperature) {
+  const double v = x / temperature;
+  return v < static_cast<double>(Limits<A>::largest) ? static_cast<A>(v) : Limits<A>::largest;
+}
+template <typename A>
+__device__ __forceinline__ A log2e_over(double temperature) {
+  return per_temperature<A>(1.4426950408889634074, temperature);
+}
 
 // x, or a finite stand-in for -inf. (For a NaN too: the exponential that it goes with is NaN.)
 template <typename A>
@@ -65,9 +77,11 @@ __device__ __forceinline__ A above_lowest(A x) {
 }
 
 // The exponent of a logit z against the largest known one, m: with c = log2(e) / T and b = m c as
-// rounded, z c - b in one operation, rounded once; b is only a point of reference, so its own rounding
-// costs nothing (4.5 instructions an element where z - m and a product made 5.5). Where m is huge, as in
-// a row masked whole with the lowest finite value, (z - m) c.
+// rounded, z c - b in one operation, rounded once (4.5 instructions an element where z - m and a product
+// made 5.5). b is only a point of reference: what its rounding moved it by, `excess`, is in every exponent
+// of the row alike and leaves the log of the sum again. That holds while it is small: past `near`, as in a
+// row masked whole with a large finite value or at a small temperature, it would take the powers out of
+// their range (by 2^440 where m c is -1.4e10), and the exponents are (z - m) c.
 template <typename A>
 struct Scale {
   A c, m, b;
@@ -75,7 +89,7 @@ struct Scale {
   __device__ __forceinline__ Scale(A m_, A c_) : c(c_), m(m_ == A(-INFINITY) ? A(0) : m_) {
 #pragma clang fp contract(off)
     b = m * c;
-    plain = b >= -Limits<A>::huge && b <= Limits<A>::huge;
+    plain = b >= -Limits<A>::near && b <= Limits<A>::near;
   }
   // What the exponents are above their exact values, in all of a row's alike.
   __device__ __forceinline__ A excess() const { return plain ? fma_of(m, c, -b) : A(0); }
@@ -88,12 +102,14 @@ template <typename A, bool ENT>
 struct Part {
   A m = A(-INFINITY), s = A(0), q = A(0);
 
-  // The sums against a larger m, whose scale is `to`.
+  // The sums against a larger m, whose scale is `to`. Their own point of reference is m c as rounded where that
+  // is near, else m c as it is, whatever the larger one's.
   __device__ __forceinline__ void move(A larger, const Scale<A>& to) {
-    // (the sums' own point of reference is m c as rounded: no contraction with the difference)
+    // (no contraction of m c with the difference)
 #pragma clang fp contract(off)
     const A own = m * to.c;
-    const A d = to.plain ? own - to.b : (m - to.m) * to.c, f = exp2_of(d);
+    const A over = own >= -Limits<A>::near && own <= Limits<A>::near ? fma_of(m, to.c, -own) : A(0);
+    const A d = (to.plain ? fma_of(m, to.c, -to.b) : (m - to.m) * to.c) - over, f = exp2_of(d);
     if constexpr (ENT) q = f * (q + s * above_lowest(d));
     s *= f;
     m = larger;
@@ -133,22 +149,6 @@ struct Part {
     if constexpr (ENT) q += q4[0];
   }
 
-  __device__ __forceinline__ void join(Part o, A c) {
-    const A larger = max_of(m, o.m);
-    const Scale<A> scale(larger, c);
-    move(larger, scale);
-    o.move(larger, scale);
-    s += o.s;
-    if constexpr (ENT) q += o.q;
-  }
-
-  __device__ __forceinline__ Part across(int d) const {
-    Part o;
-    o.m = __shfl_xor(m, d);
-    o.s = __shfl_xor(s, d);
-    if constexpr (ENT) o.q = __shfl_xor(q, d);
-    return o;
-  }
 };
 
 struct Rows {
@@ -217,9 +217,9 @@ struct Results {
   int64_t rows;
   __device__ __forceinline__ void put(int64_t r, const Part<A, ENT>& p, A zt, double temperature) const {
     constexpr A kLn2 = static_cast<A>(0.69314718055994530942);
-    const Scale<A> scale(p.m, static_cast<A>(1.4426950408889634074 / temperature));
+    const Scale<A> scale(p.m, log2e_over<A>(temperature));
     const A logs = log(p.s);
-    logp[r] = (zt - p.m) * static_cast<A>(1.0 / temperature) - (logs - scale.excess() * kLn2);
+    logp[r] = (zt - p.m) * per_temperature<A>(1.0, temperature) - (logs - scale.excess() * kLn2);
     if constexpr (ENT) entropy[r] = logs - p.q / p.s * kLn2;
     keep(r, p.m, p.s);
   }
@@ -250,13 +250,13 @@ template <int CTRL>
 __device__ __forceinline__ double dpp(double x) {
   return dpp_f64<CTRL, 0xF>(x);
 }
-// The sum, or the largest, over the G lanes of a group, in each of them: with the neighbour, the other
-// pair, then the mirrored lane of 8 and of 16 (whose quads, then halves, hold one value each).
+// The sum, or the largest, over the G lanes of a group (4 at least), in each of them: with the neighbour, the
+// other pair, then the mirrored lane of 8 and of 16 (whose quads, then halves, hold one value each).
 template <int G, typename A, typename Op>
 __device__ __forceinline__ A over_group(A x, Op op) {
   x = op(x, dpp<0xB1>(x));   // quad_perm 1 0 3 2
   x = op(x, dpp<0x4E>(x));   // quad_perm 2 3 0 1
-  x = op(x, dpp<0x141>(x));  // row_half_mirror
+  if constexpr (G > 4) x = op(x, dpp<0x141>(x));  // row_half_mirror
   if constexpr (G > 8) x = op(x, dpp<0x140>(x));  // row_mirror
   if constexpr (G > 16) x = op(x, __shfl_xor(x, 16));
   if constexpr (G > 32) x = op(x, __shfl_xor(x, 32));
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_short_kernel(const T* __res
   const bool some = r < out.rows;
   const int64_t t = some ? targets[r] : ignore;
   const bool kept = t != ignore;
-  const A c = static_cast<A>(1.4426950408889634074 / temperature);
+  const A c = log2e_over<A>(temperature);
   const T* z = logits + (kept ? where.at(r) : 0);
   const int whole = vocab / kN;
   typename Vec<T>::type v[U];
@@ -331,11 +331,20 @@ __global__ __launch_bounds__(kThreads) void logprobs_short_kernel(const T* __res
   else out.put_ignored(r);
 }
 
-// The sums over the 64 lanes of each wave, then over the workgroup's waves, in wave 0's lanes.
+// The parts of a group of G lanes joined, in each of them: moved to the largest of all, then summed.
+template <int G, typename A, bool ENT>
+__device__ __forceinline__ void join_group(Part<A, ENT>& p, A c) {
+  auto plus = [](A a, A b) { return a + b; };
+  const A larger = over_group<G>(p.m, [](A a, A b) { return max_of(a, b); });
+  p.move(larger, Scale<A>(larger, c));
+  p.s = over_group<G>(p.s, plus);
+  if constexpr (ENT) p.q = over_group<G>(p.q, plus);
+}
+
+// The parts of each wave's 64 lanes, then of the workgroup's waves.
 template <int NT, typename A, bool ENT>
 __device__ __forceinline__ void join_all(Part<A, ENT>& p, A c) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) p.join(p.across(d), c);
+  join_group<64>(p, c);
   if constexpr (NT > 64) {
     constexpr int kWaves = NT / 64;
     __shared__ A parts[3][kWaves];
@@ -349,8 +358,7 @@ __device__ __forceinline__ void join_all(Part<A, ENT>& p, A c) {
     p.m = parts[0][threadIdx.x % kWaves];
     p.s = parts[1][threadIdx.x % kWaves];
     if constexpr (ENT) p.q = parts[2][threadIdx.x % kWaves];
-#pragma unroll
-    for (int d = kWaves / 2; d > 0; d >>= 1) p.join(p.across(d), c);
+    join_group<kWaves>(p, c);
   }
 }
 
@@ -372,7 +380,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const T* __restrict__ logi
     if (threadIdx.x == 0 && blockIdx.y == 0) out.put_ignored(r);
     return;
   }
-  const A c = static_cast<A>(1.4426950408889634074 / temperature);
+  const A c = log2e_over<A>(temperature);
   const T* z = logits + where.at(r);
   const A zt = threadIdx.x == 0 ? at_target(z, t, vocab) : A(0);
   Part<A, ENT> p;
@@ -427,7 +435,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
   const int64_t r = blockIdx.x;
   const int64_t t = targets[r];
   if (t == ignore) return;
-  const A c = static_cast<A>(1.4426950408889634074 / temperature);
+  const A c = log2e_over<A>(temperature);
   Part<A, ENT> p;
   if (static_cast<int>(threadIdx.x) < count) p = parts[r * count + threadIdx.x];
   const A zt = threadIdx.x == 0 ? at_target(logits + where.at(r), t, vocab) : A(0);
@@ -463,18 +471,21 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(
   const bool kept = target != ignore, in = target >= 0 && target < vocab;
   const int t = in ? static_cast<int>(target) : -kN;
   const T* z = logits + (kept ? where.at(r) : 0);
-  const A c = static_cast<A>(1.4426950408889634074 / temperature), inv = static_cast<A>(1.0 / temperature);
+  const A c = log2e_over<A>(temperature), inv = per_temperature<A>(1.0, temperature);
   const Scale<A> scale(stats[r], c);
   const A s = stats[rows + r];
   const A gr = !in ? quiet_nan<A>() : (g != nullptr ? g[r] * inv : A(0));
-  // d_j = e_j (a + b x_j), and gr more at the target
+  // d_j = e_j a + (e_j x_j) b, and gr more at the target (e_j x_j first: zero times a large b)
   A a = -gr / s, b = A(0);
   if constexpr (ENT) {
     const A gh = ge[r] * inv;
     a -= gh * (entropy[r] - log(s)) / s;
     b = -gh * static_cast<A>(0.69314718055994530942) / s;
   }
-  auto of = [&](A x) { return exp2_of(x) * (ENT ? a + b * above_lowest(x) : a); };
+  auto of = [&](A x) {
+    const A e = exp2_of(x);
+    return ENT ? fma_of(e * above_lowest(x), b, e * a) : e * a;
+  };
   auto of_one = [&](A v) { return of(scale.plain ? fma_of(v, c, -scale.b) : (v - scale.m) * c); };
   auto put = [&](int start, typename Vec<T>::type v) {
     A d[kN];
