@@ -110,3 +110,60 @@ def test_saved_tensors_of_another_size_are_refused() -> None:
                 torch.autograd.grad(loss, z, retain_graph=True)
             with pytest.raises(RuntimeError, match="came back|must match|must be"):
                 torch.autograd.grad(loss, z, retain_graph=True)
+
+
+def test_forward_mode_is_refused() -> None:
+    """Without a forward derivative, a call on a dual tensor raises: a result without a tangent would read as a
+    derivative of zero."""
+    from torch.autograd import forward_ad
+
+    gen = torch.Generator().manual_seed(2)
+    logits, t = torch.randn(5, 40, generator=gen).cuda(), torch.zeros(5, dtype=torch.int64, device="cuda")
+    x, old, adv = torch.randn(4, 30, generator=gen).cuda(), torch.randn(4, 30, generator=gen).cuda(), torch.ones(4).cuda()
+    calls = {
+        "logprobs": lambda d: token_logprobs(d(logits), t),
+        "logprobs with entropy": lambda d: token_logprobs(d(logits), t, entropy=True),
+        "preference": lambda d: preference_loss(d(x), old),
+        "preference, none": lambda d: preference_loss(d(x), reduction="none"),
+        "preference, the reference's": lambda d: preference_loss(x, d(old)),
+        "preference, half": lambda d: preference_loss(d(x.half())),
+        "policy": lambda d: policy_loss(d(x), old, adv),
+        "policy, the old ones'": lambda d: policy_loss(x, d(old), adv),
+        "policy, advantages": lambda d: policy_loss(x, old, d(adv)),
+        "policy, the reference's": lambda d: policy_loss(x, old, adv, reference_logps=d(old), kl_coef=0.1),
+    }
+    constants = {n for n in calls if "'" in n or "advantages" in n}
+    for name, call in calls.items():
+        # (tensors that get no gradient may not require one)
+        for tracked in (False,) if name in constants else (False, True):
+            for no_grad in (False, True):
+                say(f"forward mode: {name}, {tracked=}, {no_grad=}")
+                with forward_ad.dual_level(), torch.set_grad_enabled(not no_grad):
+                    with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+                        call(lambda v: forward_ad.make_dual(v.clone().requires_grad_(tracked), torch.ones_like(v)))
+        call(lambda v: v)  # (and none of it outside)
+
+
+def test_function_transforms() -> None:
+    gen = torch.Generator().manual_seed(3)
+    logits, t = torch.randn(5, 40, generator=gen).cuda(), torch.zeros(5, dtype=torch.int64, device="cuda")
+    x, adv = torch.randn(4, 30, generator=gen).cuda(), torch.ones(4).cuda()
+    calls = {
+        "logprobs": (lambda z: token_logprobs(z, t).sum(), logits),
+        "preference": (lambda z: preference_loss(z).loss, x),
+        "policy": (lambda z: policy_loss(z, x, adv).loss, x),
+    }
+    for name, (call, value) in calls.items():
+        say(f"transforms: {name}")
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (value,), (torch.ones_like(value),))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(call)(value)
+        # (a map over a batch: one call after another, with their gradients)
+        z = torch.stack([value, 0.5 * value]).requires_grad_()
+        out = torch.func.vmap(call)(z)
+        (grad,) = torch.autograd.grad(out.sum(), z)
+        for i in range(2):
+            one = z[i].detach().requires_grad_()
+            want = call(one)
+            assert torch.equal(out[i], want) and torch.equal(grad[i], torch.autograd.grad(want, one)[0])

@@ -12,12 +12,14 @@
 // torch's current one, and the C ABI of libtorchisotonic_amd.so does the work. Nothing here waits for
 // the GPU.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 
@@ -57,6 +59,16 @@ void once(const char* what) {
 
 // Whether a backward may follow (asked outside the autograd node's forward, which runs untracked).
 bool tracked(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+
+// There are no forward-mode derivatives: a dual tensor raises, whether it requires a gradient or not, as its result
+// without a tangent would read as a derivative of zero.
+void no_tangents(std::initializer_list<const at::Tensor*> tensors, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(t == nullptr || !t->defined() || !t->_fw_grad(0).defined(), "torchisotonic_amd.", what,
+                " has no forward-mode derivative (jvp)");
+}
+const at::Tensor* some(const std::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 // A saved tensor as the kernels take it. (What comes back is what saved-tensor hooks made of it: a copy, maybe in
 // another layout, so that nothing of the layout it was saved in holds.)
@@ -181,6 +193,7 @@ struct LogprobsFn : public torch::autograd::Function<LogprobsFn> {
 // (the entropy undefined, in Python None, where not wanted)
 std::tuple<at::Tensor, at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& targets,
                                                   double temperature, int64_t ignore_index, bool entropy) {
+  no_tangents({&logits}, "token_logprobs");
   if (!tracked(logits)) {
     const Logprobs out = logprobs_of(logits, targets, temperature, ignore_index, entropy, false);
     return {out.logp, out.entropy};
@@ -303,6 +316,7 @@ struct PreferenceFn : public torch::autograd::Function<PreferenceFn> {
 Three preference_loss(const at::Tensor& logps, const std::optional<at::Tensor>& ref,
                       const std::optional<at::Tensor>& offsets, const std::optional<at::Tensor>& mask, int64_t kind,
                       double beta, double smoothing, bool average, int64_t reduction) {
+  no_tangents({&logps, some(ref)}, "preference_loss");
   if (!tracked(logps)) {
     const Preference out = preference_of(logps, ref, offsets, mask, kind, beta, smoothing, average, reduction, false);
     return {out.loss, out.rewards[0], out.rewards[1]};
@@ -320,11 +334,11 @@ struct PolicyCall {
 
   // The sequences, once every tensor is checked.
   Sequences checked() const {
-    auto some = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
-    const Sequences s = sequences_of(logps, some(offsets), "policy_loss");
+    auto maybe = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+    const Sequences s = sequences_of(logps, maybe(offsets), "policy_loss");
     check_like(logps, old, logps.scalar_type(), "old_logps", "policy_loss");
-    check_like(logps, some(ref), logps.scalar_type(), "reference_logps", "policy_loss");
-    check_like(logps, some(mask), at::kBool, "mask", "policy_loss");
+    check_like(logps, maybe(ref), logps.scalar_type(), "reference_logps", "policy_loss");
+    check_like(logps, maybe(mask), at::kBool, "mask", "policy_loss");
     TORCH_CHECK((advantages.sizes() == logps.sizes() || (advantages.dim() == 1 && advantages.numel() == s.count)) &&
                     advantages.device() == logps.device() && advantages.scalar_type() == logps.scalar_type() &&
                     advantages.is_contiguous(),
@@ -415,6 +429,7 @@ Three policy_loss(const at::Tensor& logps, const at::Tensor& old, const at::Tens
                   const std::optional<at::Tensor>& ref, const std::optional<at::Tensor>& offsets,
                   const std::optional<at::Tensor>& mask, double clip_low, double clip_high, double kl_coef,
                   int64_t reduction) {
+  no_tangents({&logps, &old, &advantages, some(ref)}, "policy_loss");
   const variable_list out = PolicyFn::apply(logps, old, advantages, ref, offsets, mask, clip_low, clip_high, kl_coef,
                                             reduction, tracked(logps));
   const at::NoGradGuard untracked;

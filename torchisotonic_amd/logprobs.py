@@ -37,8 +37,8 @@ def token_logprobs(
     """The log-probability of each target token: ``log_softmax(logits / temperature)`` at
     ``targets``, for logits [..., vocab] (float32, float64, bfloat16 or float16, on the GPU) and
     integer targets [...]; with ``entropy`` the rows' entropies (in nats) as well. Results are
-    float32 (float64 for float64 logits) and differentiable in the logits, whose gradient has their
-    dtype.
+    float32 (float64 for float64 logits) and differentiable in the logits (once, in reverse mode), whose
+    gradient has their dtype.
 
     A row whose target is ``ignore_index`` (a prompt's or a pad's) gives 0 with a gradient of 0,
     and its logits are not read, whatever they hold. To score a text against itself shifted by one,
