@@ -474,8 +474,9 @@ int ti_logprobs_bwd(const void* logits, const int64_t* targets, const void* stat
  * end to end with offsets (sequences + 1 device int64 values, from 0 to total, not decreasing) or, with
  * offsets NULL, of `len` places each (total = sequences * len). mask (one byte a token, or NULL): a
  * token whose byte is 0 counts as absent and its values are not used. Offsets are clamped as they are
- * read, so no access leaves the arrays; offsets that are not as described make the loss NaN (with
- * TI_REDUCE_NONE the losses of the pairs whose own they are; the other pairs' may then be anything).
+ * read, so no access leaves the arrays; offsets that are not as described make the loss and every
+ * unmasked token's gradient NaN (with TI_REDUCE_NONE the losses and slopes of the pairs whose own they
+ * are; the other pairs' may then be anything).
  *
  * Preference: the first half of the sequences are the chosen ones, the second half the rejected ones of
  * the same pairs. With s the sum over a sequence's tokens of logps - ref (ref NULL: of logps), or their

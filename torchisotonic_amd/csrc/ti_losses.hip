@@ -192,6 +192,17 @@ __device__ __forceinline__ double block_sum(double v) {
   return s[0];
 }
 
+// The same, and whether any thread's `any` was set, in every thread.
+template <int NT>
+__device__ __forceinline__ double block_sum(double v, bool& any) {
+  __shared__ int flag[NT / 64];
+  const bool wave = __any(any);
+  if ((threadIdx.x & 63) == 0) flag[threadIdx.x >> 6] = wave;
+  v = block_sum<NT>(v);  // (whose barriers come between)
+  any = __any(flag[threadIdx.x % (NT / 64)]);
+  return v;
+}
+
 // Four consecutive values of a token array at any alignment; those past the end zero.
 template <typename T>
 struct Four {
@@ -362,7 +373,7 @@ __device__ __forceinline__ double group_sum(double v) {
   return v;
 }
 
-// The sum of sequence i, by G lanes, in the last of them.
+// The sum of sequence i, by G lanes, in the last of them; NaN of -1 where its offsets are not sound.
 template <int G>
 __device__ __forceinline__ Sum sum_of(const Sequences& seq, int64_t i, int tile_places, const Sum* __restrict__ first,
                                       const Sum* __restrict__ last, const Sum* __restrict__ whole) {
@@ -372,8 +383,22 @@ __device__ __forceinline__ Sum sum_of(const Sequences& seq, int64_t i, int tile_
   if (a < b) {
     const int64_t t0 = a / tile_places, t1 = (b - 1) / tile_places;
     if (lane == 0) v = a == t0 * tile_places ? first[t0] : (b < (t0 + 1) * tile_places ? whole[i] : last[t0]);
-#pragma unroll 8
-    for (int64_t t = t0 + 1 + lane; t <= t1; t += G) {
+    // (eight on their way at a time, which the compiler's own schedule does not keep: two sequences of 8 million
+    // tokens in 52.7 us, one after another 162 us)
+    constexpr int kAhead = 8;
+    int64_t t = t0 + 1 + lane;
+    for (; t + (kAhead - 1) * G <= t1; t += kAhead * G) {
+      Sum w[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) w[i] = first[t + i * G];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        v.s += w[i].s;
+        v.n += w[i].n;
+      }
+    }
+    for (; t <= t1; t += G) {
       const Sum w = first[t];
       v.s += w.s;
       v.n += w.n;
@@ -381,7 +406,7 @@ __device__ __forceinline__ Sum sum_of(const Sequences& seq, int64_t i, int tile_
   }
   v.s = group_sum<G>(v.s);
   v.n = group_sum<G>(v.n);
-  if (!seq.sound(i)) v.s = quiet_nan<double>();
+  if (!seq.sound(i)) v = Sum{quiet_nan<double>(), -1.0};
   return v;
 }
 
@@ -436,11 +461,11 @@ struct PairArgs {
 //
 // The pairs from `begin` on, G lanes a sequence and 2 G a pair (the chosen sequence by the first half, the
 // rejected one by the second), `step` pairs apart: their results, and the sum of their losses in this
-// workgroup.
+// workgroup, and whether it met offsets that are not sound.
 template <int NT, int G, typename T>
 __device__ __forceinline__ double pair_losses(const Sequences& seq, int64_t begin, int64_t step, int tile_places,
                                               const Sum* __restrict__ first, const Sum* __restrict__ last,
-                                              const Sum* __restrict__ whole, const PairArgs<T>& a) {
+                                              const Sum* __restrict__ whole, const PairArgs<T>& a, bool& bad) {
   const int64_t pairs = seq.count / 2;
   const int lane = threadIdx.x & 63, side = (lane / G) & 1;
   const double scale = a.scale(pairs);
@@ -452,6 +477,7 @@ __device__ __forceinline__ double pair_losses(const Sequences& seq, int64_t begi
     const int at = lane / (2 * G) * (2 * G) + G - 1;  // (the chosen one's last lane; the rejected one's G on)
     const Sum c{__shfl(mine.s, at), __shfl(mine.n, at)}, j{__shfl(mine.s, at + G), __shfl(mine.n, at + G)};
     if (!in || lane % (2 * G) != 0) continue;
+    bad = bad || c.n < 0.0 || j.n < 0.0;
     const double wc = a.average && c.n > 0.0 ? 1.0 / c.n : 1.0, wj = a.average && j.n > 0.0 ? 1.0 / j.n : 1.0;
     const double sc = c.s * wc, sj = j.s * wj;
     const Pair v = pair_loss(sc - sj, a.kind, a.beta, a.smoothing);
@@ -464,22 +490,39 @@ __device__ __forceinline__ double pair_losses(const Sequences& seq, int64_t begi
     if (a.reduction == TI_REDUCE_NONE) a.loss[p] = static_cast<T>(v.loss);
     all += v.loss;
   }
-  return a.reduction == TI_REDUCE_NONE ? 0.0 : block_sum<NT>(all);
+  return a.reduction == TI_REDUCE_NONE ? 0.0 : block_sum<NT>(all, bad);
 }
+
+// Offsets that are not sound leave no token with a gradient to go by: every slope NaN, by one workgroup, all of
+// whose threads have the same `bad`.
+template <int NT, typename T>
+__device__ __forceinline__ void void_slopes(bool bad, T* __restrict__ slopes, int64_t count) {
+  if (!bad || slopes == nullptr) return;
+  for (int64_t i = threadIdx.x; i < count; i += NT) slopes[i] = quiet_nan<T>();
+}
+
+// A workgroup's sum of its pairs' losses, and whether it met offsets that are not sound.
+struct PairPart {
+  double all;
+  int64_t bad;
+};
 
 template <typename T, int G>
 __global__ __launch_bounds__(kPairThreads) void preference_pairs_kernel(Sequences seq, int tile_places,
                                                                         const Sum* __restrict__ first,
                                                                         const Sum* __restrict__ last,
                                                                         const Sum* __restrict__ whole, PairArgs<T> a,
-                                                                        double* __restrict__ parts) {
+                                                                        PairPart* __restrict__ parts) {
   constexpr int kEach = 32 / G;  // pairs a wave
   const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kPairThreads / 64) + (threadIdx.x >> 6);
+  bool bad = false;
   const double all = pair_losses<kPairThreads, G>(seq, wave * kEach, static_cast<int64_t>(gridDim.x) * (kPairThreads / 64) * kEach,
-                                                  tile_places, first, last, whole, a);
-  if (threadIdx.x != 0 || a.reduction == TI_REDUCE_NONE) return;
+                                                  tile_places, first, last, whole, a, bad);
+  if (a.reduction == TI_REDUCE_NONE) return;
+  if (gridDim.x == 1) void_slopes<kPairThreads>(bad, a.slopes, seq.count);
+  if (threadIdx.x != 0) return;
   if (gridDim.x == 1) a.loss[0] = static_cast<T>(all * a.scale(seq.count / 2));
-  else parts[blockIdx.x] = all;
+  else parts[blockIdx.x] = PairPart{all, bad};
 }
 
 // Few tokens in one workgroup: their sums, then the pairs. (Four pairs, 2620 tokens: 6.2 us, in two
@@ -494,16 +537,26 @@ __global__ __launch_bounds__(kPairThreads) void preference_small_kernel(const T*
   for (int64_t tile = threadIdx.x >> 6; tile * 256 < seq.total; tile += kEach)
     tile_sums<T, 1>(logps, ref, mask, seq, tile, heads[threadIdx.x >> 6], first, last, whole);
   __syncthreads();
-  const double all = pair_losses<kPairThreads, 32>(seq, threadIdx.x >> 6, kEach, 256, first, last, whole, a);
-  if (threadIdx.x == 0 && a.reduction != TI_REDUCE_NONE) a.loss[0] = static_cast<T>(all * a.scale(seq.count / 2));
+  bool bad = false;
+  const double all = pair_losses<kPairThreads, 32>(seq, threadIdx.x >> 6, kEach, 256, first, last, whole, a, bad);
+  if (a.reduction == TI_REDUCE_NONE) return;
+  void_slopes<kPairThreads>(bad, a.slopes, seq.count);
+  if (threadIdx.x == 0) a.loss[0] = static_cast<T>(all * a.scale(seq.count / 2));
 }
 
 template <typename T>
-__global__ __launch_bounds__(kPairThreads) void preference_mean_kernel(const double* __restrict__ parts, int count,
-                                                                   double scale, T* __restrict__ loss) {
+__global__ __launch_bounds__(kPairThreads) void preference_mean_kernel(const PairPart* __restrict__ parts, int count,
+                                                                       double scale, T* __restrict__ loss,
+                                                                       T* __restrict__ slopes, int64_t sequences) {
   double all = 0.0;
-  for (int i = threadIdx.x; i < count; i += kPairThreads) all += parts[i];
-  all = block_sum<kPairThreads>(all);
+  bool bad = false;
+  for (int i = threadIdx.x; i < count; i += kPairThreads) {
+    const PairPart part = parts[i];
+    all += part.all;
+    bad = bad || part.bad != 0;
+  }
+  all = block_sum<kPairThreads>(all, bad);
+  void_slopes<kPairThreads>(bad, slopes, sequences);
   if (threadIdx.x == 0) loss[0] = static_cast<T>(all * scale);
 }
 
@@ -888,6 +941,22 @@ __device__ __forceinline__ PolicySums policy_sums(const PolicyPart& v, bool bad)
   return all;
 }
 
+// Offsets that are not sound leave no token with a gradient to go by: that of every unmasked one NaN, by one
+// workgroup. (Written once the pass that wrote gradients is over, so that it costs the others nothing.)
+template <int NT, typename T>
+__device__ __forceinline__ void void_gradient(const uint8_t* __restrict__ mask, int64_t total, T* __restrict__ grad) {
+  if (grad == nullptr) return;
+#pragma unroll 4
+  for (int64_t j = static_cast<int64_t>(threadIdx.x) * 4; j < total; j += NT * 4) {
+    Four<uint8_t> m{{1, 1, 1, 1}};
+    if (mask != nullptr) m.load(mask, j, total);
+    Four<T> d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d.v[i] = m.v[i] != 0 ? quiet_nan<T>() : T(0);
+    d.store(grad, j, total);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void put_policy(const PolicySums& v, T* loss, T* kl, T* cut) {
   const double per = 1.0 / (v.n < 1.0 ? 1.0 : v.n);
@@ -918,7 +987,8 @@ __global__ __launch_bounds__(kThreads) void policy_kernel(PolicyInputs<T> in, Se
 template <typename T>
 __global__ __launch_bounds__(kPairThreads) void policy_join_kernel(const PolicySums* __restrict__ sums, int count,
                                                                    T* __restrict__ loss, T* __restrict__ kl,
-                                                                   T* __restrict__ cut) {
+                                                                   T* __restrict__ cut, const uint8_t* __restrict__ mask,
+                                                                   int64_t total, T* __restrict__ grad) {
   double v[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 8
   for (int i = threadIdx.x; i < count; i += kPairThreads) {
@@ -929,6 +999,7 @@ __global__ __launch_bounds__(kPairThreads) void policy_join_kernel(const PolicyS
     v[3] += s.n;
   }
   block_sums<kPairThreads>(v);
+  if (!(v[3] >= 0.0)) void_gradient<kPairThreads>(mask, total, grad);
   if (threadIdx.x == 0) put_policy(PolicySums{v[0], v[1], v[2], v[3]}, loss, kl, cut);
 }
 
@@ -948,8 +1019,10 @@ __global__ __launch_bounds__(kCountThreads) void policy_small_kernel(PolicyInput
   __shared__ __attribute__((aligned(16))) int heads[kCountThreads / 64][256];
   for (int64_t begin = (threadIdx.x >> 6) * 256; begin < seq.total; begin += kCountThreads / 64 * 256)
     policy_places<T, 1>(in, seq, begin, heads[threadIdx.x >> 6], weight, nullptr, 0, in.mask != nullptr ? weights : nullptr, v);
-  const PolicySums all = policy_sums<kCountThreads>(v, unsound(seq, threadIdx.x, kCountThreads));
+  const bool bad = unsound(seq, threadIdx.x, kCountThreads);
+  const PolicySums all = policy_sums<kCountThreads>(v, bad);
   if (threadIdx.x == 0) put_policy(all, loss, kl, cut);
+  if (seq.offsets != nullptr && __syncthreads_or(bad) != 0) void_gradient<kCountThreads>(in.mask, seq.total, in.grad);
 }
 
 // grad times g; a g of one leaves it as it is.
@@ -1007,14 +1080,14 @@ struct Carve {
 };
 struct PreferenceWork {
   Sum *first, *last, *whole;
-  double* parts;
+  PairPart* parts;
   size_t bytes;
   PreferenceWork(void* work, int64_t total, int64_t sequences) {
     Carve c{static_cast<char*>(work)};
     first = c.take<Sum>(tiles_of(total));
     last = c.take<Sum>(tiles_of(total));
     whole = c.take<Sum>(sequences);
-    parts = c.take<double>(kPairBlocks);
+    parts = c.take<PairPart>(kPairBlocks);
     bytes = c.used;
   }
 };
@@ -1062,7 +1135,8 @@ hipError_t preference(const PreferenceArgs& a, void* work) {
                                                                                     w.last, w.whole, pa, w.parts);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || blocks == 1 || a.reduction == TI_REDUCE_NONE) return e;
     preference_mean_kernel<T><<<dim3(1), dim3(kPairThreads), 0, a.stream>>>(
-        w.parts, static_cast<int>(blocks), a.reduction == TI_REDUCE_MEAN ? 1.0 / static_cast<double>(pairs) : 1.0, pa.loss);
+        w.parts, static_cast<int>(blocks), a.reduction == TI_REDUCE_MEAN ? 1.0 / static_cast<double>(pairs) : 1.0, pa.loss,
+        pa.slopes, seq.count);
     return hipGetLastError();
   };
   return a.dtype == TI_F32 ? go(float{}) : go(double{});
@@ -1117,7 +1191,8 @@ hipError_t policy(const PolicyArgs& a, void* work) {
     kernel<<<dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, a.stream>>>(
         in, seq, weight, mean && blocks > 0 ? w.tokens : nullptr, blocks, blocks > 0 ? w.weights : nullptr, w.sums);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    policy_join_kernel<T><<<dim3(1), dim3(kPairThreads), 0, a.stream>>>(w.sums, static_cast<int>(tiles), loss, kl, cut);
+    policy_join_kernel<T><<<dim3(1), dim3(kPairThreads), 0, a.stream>>>(w.sums, static_cast<int>(tiles), loss, kl, cut, in.mask,
+                                                                         seq.total, in.grad);
     return hipGetLastError();
   };
   return a.dtype == TI_F32 ? go(float{}) : go(double{});

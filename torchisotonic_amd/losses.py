@@ -15,8 +15,8 @@ pads), whatever their values. ``token_logprobs`` gives the log-probabilities.
 
 The tokens' sums, the losses and the gradients run in HIP kernels (``ti_preference``, ``ti_policy``);
 sums are float64 in a fixed order. Nothing waits for the GPU: offsets on the GPU that are not what they
-have to be make the loss NaN instead of raising (of single losses, the pairs' whose own they are: no
-other can then be relied on). The reference has no counterpart.
+have to be make the loss and the gradient of every unmasked token NaN instead of raising (of single
+losses, the pairs' whose own they are: no other can then be relied on). The reference has no counterpart.
 """
 
 from __future__ import annotations
