@@ -1172,7 +1172,7 @@ hipError_t policy(const PolicyArgs& a, void* work) {
     }
     const bool mean = a.reduction == TI_REDUCE_MEAN, by_sequence = a.reduction == TI_REDUCE_SEQUENCES;
     int blocks = 0;
-    if (a.mask != nullptr && (mean || by_sequence)) {
+    if (seq.total > 0 && a.mask != nullptr && (mean || by_sequence)) {
       // masked sequences counted by as many threads as their length asks for (20000 of 1 to 600 tokens, the policy
       // loss: by 8 threads each 35.7 us, by 64 41.7 us; 8000 of 1 to 2000: 49.3 and 45.2 us); else the places in turn
       const int64_t length = seq.total / seq.count;
