@@ -117,3 +117,18 @@ def test_values_that_are_nan_leave_other_gradients() -> None:
         own = torch.zeros(total, dtype=torch.bool, device="cuda")
         own[last:] = own[lo:hi] = True
         assert bool(grad[own].isnan().all()) and bool(grad[~own].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", ["offsets", "lengths"])
+@pytest.mark.parametrize("place", ["cpu", "cuda"])
+def test_tokens_of_no_sequence_are_refused(kind: str, place: str) -> None:
+    """What the number of offsets alone says is wrong needs no waiting."""
+    x = torch.zeros(10, device="cuda", requires_grad=True)
+    none = torch.zeros(1 if kind == "offsets" else 0, dtype=torch.int64, device=place)
+    for call in (lambda: preference_loss(x, **{kind: none}), lambda: policy_loss(x, x.detach(), x.detach(), **{kind: none}),
+                 lambda: policy_loss(x, x.detach(), x.detach()[:0], **{kind: none}, reduction="sequence_mean")):
+        with pytest.raises(ValueError, match="offsets must run from 0"):
+            call()
+    empty = x[:0]
+    assert float(preference_loss(empty, **{kind: none}).loss) == 0.0
+    assert float(policy_loss(empty, empty.detach(), empty.detach(), **{kind: none}).loss) == 0.0

@@ -218,6 +218,8 @@ Sequences sequences_of(const at::Tensor& logps, const std::optional<at::Tensor>&
                     offsets->scalar_type() == at::kLong && offsets->is_contiguous() &&
                     offsets->device() == logps.device(),
                 "torchisotonic_amd.", what, ": offsets must be 1-D int64, contiguous, on logps' device, with 1-D logps");
+    TORCH_CHECK(offsets->numel() > 1 || logps.numel() == 0, "torchisotonic_amd.", what, ": offsets must run from 0 to ",
+                logps.numel());
     return {logps.numel(), offsets->numel() - 1, 0, offsets->data_ptr<int64_t>()};
   }
   if (logps.dim() == 1) return {logps.numel(), 1, logps.numel(), nullptr};

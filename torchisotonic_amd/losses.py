@@ -105,7 +105,10 @@ def _sequences(logps: Tensor, offsets, lengths) -> Tensor | None:
         if int(host[0]) != 0 or int(host[-1]) != logps.numel():
             raise ValueError(f"offsets must run from 0 to logps.numel() = {logps.numel()}")
         offsets, lengths = host, None
-    return _offsets_tensor(offsets, lengths, logps.device)
+    off = _offsets_tensor(offsets, lengths, logps.device)
+    if off.numel() == 1 and logps.numel() > 0:
+        raise ValueError(f"offsets must run from 0 to logps.numel() = {logps.numel()}")
+    return off
 
 
 def preference_loss(
