@@ -499,8 +499,8 @@ int ti_logprobs_bwd(const void* logits, const int64_t* targets, const void* stat
  * multiplies it by g (one value), in place.
  *
  * The *_workspace functions give the bytes of device workspace (256-byte aligned) that the forward
- * functions need. Sums run in float64, in a fixed order. sequences stay below 2^26 and total below
- * 2^33.
+ * functions need. Sums run in float64, in a fixed order, but that the policy's first adds four float32
+ * tokens' terms in float32. sequences stay below 2^26 and total below 2^33.
  */
 #define TI_LOSS_LOGISTIC 0
 #define TI_LOSS_HINGE 1

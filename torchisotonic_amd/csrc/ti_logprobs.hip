@@ -264,7 +264,7 @@ __device__ __forceinline__ A over_group(A x, Op op) {
 }
 
 // Bound by its vector instructions and the latency of a wave's few loads: 65536 rows of 257 float16 (34 MB)
-// in 8.6 us, 3.9 TB/s; 32768 of 2000 bfloat16 (131 MB) in 25 us, 5.2 TB/s. (With a running maximum and
+// in 9.1 us, 3.8 TB/s; 32768 of 2000 bfloat16 (131 MB) in 25 us, 5.2 TB/s. (With a running maximum and
 // joins across the lanes, as the long rows have, 13.2 and 33 us.)
 //
 // Short rows, G lanes each, whole in registers: U vectors a lane and the elements past the last whole
@@ -363,7 +363,7 @@ __device__ __forceinline__ void join_all(Part<A, ENT>& p, A c) {
 }
 
 // Bound by its reads: 8192 rows of 128000 bfloat16 (2.1 GB) in 329 us, 6.4 TB/s, above a copy's rate; 256
-// rows, one a compute unit, in 15.4 us, 4.3 TB/s, of which the exponentials' instructions are about 8 us.
+// rows, one a compute unit, in 15.1 us, 4.3 TB/s, of which the exponentials' instructions are about 7 us.
 //
 // Long rows, NT threads each (rows of at least three vectors). With `parts`, workgroup (r, y) takes the
 // y-th of gridDim.y stretches of the row and leaves its sums there.
@@ -458,11 +458,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_grad_kernel(
   using A = typename AccOf<T>::type;
   constexpr int kN = Vec<T>::kN;
   const int lane = threadIdx.x % G;
-  // (from the last row on: the forward's last rows are the ones still in the last-level cache)
   // (a row's chunks one after another, so that what is read and written together lies together: chunk by
   // chunk over all rows took 822 us where this takes 695 us, 8192 rows of 128000 bfloat16)
   const unsigned chunk = G >= kThreads ? blockIdx.x % chunks : 0;
   unsigned block = G >= kThreads ? blockIdx.x / chunks : blockIdx.x;
+  // (rows from both ends in turn: the forward's last ones are still in the last-level cache)
   if (mixed) block = block % 2 == 0 ? gridDim.x / chunks - 1 - block / 2 : block / 2;
   const int64_t r = static_cast<int64_t>(block) * (kThreads / G) + threadIdx.x / G;
   if (r >= rows) return;
@@ -559,9 +559,9 @@ int64_t grad_chunks(int64_t vectors) {
 }
 
 // Stretches a row is read in: one, but for a few rows of 65536 logits or more, whose exponentials are
-// more work than one compute unit's share of the read (a row of 128000 bfloat16 by 1024 threads: 8.9 us;
-// by 15 workgroups and a second launch that joins them: 5.5 us; 64 rows: 10.1 and 9.1 us; 128 rows: 10.7
-// and 11.3 us; one row of 32000: 4.8 and 5.3 us).
+// more work than one compute unit's share of the read (a row of 128000 bfloat16 by 1024 threads: 8.3 us;
+// by 15 workgroups and a second launch that joins them: 5.3 us; 64 rows: 9.8 and 8.9 us; 128 rows: 10.4
+// and 11.2 us; one row of 32000: 4.5 and 5.5 us; where both limits meet, 64 rows of 70000, 6.3 and 7.5 us).
 int64_t stretches(int64_t rows, int64_t vocab) {
   if (rows > 64 || vocab < 65536) return 1;
   const int64_t want = 512 / (rows > 0 ? rows : 1), most = vocab / 8192;
@@ -621,8 +621,8 @@ hipError_t logprobs(const LogprobArgs& a, void* work) {
     };
     // (eight to sixteen vectors a thread, so that a row's start and its joining are little of its time and
     // a CU has several rows on the way; few rows by as many threads as there are. bfloat16: 8192 rows of
-    // 128000 in 350, 343 and 329 us by 256, 512 and 1024 threads, 2048 of 50001 in 38.5, 37.3 and 41.0 us,
-    // 8192 of 16000 in 51, 60 and 85 us; 16384 of 5000 by 64 threads 33 us, by 256 46 us)
+    // 128000 in 351, 343 and 330 us by 256, 512 and 1024 threads, 2048 of 50001 in 37.8, 36.6 and 40.4 us,
+    // 8192 of 16000 in 50, 55 and 70 us; 16384 of 5000 by 64 threads 33 us, by 256 45 us)
     if (n > 1) go(logprobs_kernel<T, ENT, 256>, 256);
     else if (a.rows <= 512 || vectors > 12000) go(logprobs_kernel<T, ENT, 1024>, 1024);
     else if (vectors > 4096) go(logprobs_kernel<T, ENT, 512>, 512);

@@ -3,7 +3,8 @@
 //
 // The tokens of sequence i are those of the places [start(i), start(i + 1)) of the packed arrays, given
 // by offsets or, for rows of one length, by i times that length; a masked token counts as absent,
-// whatever its values. Sums run in float64.
+// whatever its values. Sums run in float64; the policy loss's terms are of the tokens' type, and the first
+// four of float32 are added in it.
 //
 // Preference: with x = l - l_ref, s_i the sum of x over the sequence's tokens (or their mean; 0 where
 // there are none), the first half of the sequences chosen and the second half rejected, and
@@ -455,7 +456,7 @@ struct PairArgs {
 };
 
 // Bound by latency: a chain of three reads (a sequence's starts, its parts, its pair's other half) and the
-// scalar formula (1024 pairs, one a wave: 6.6 us). Sequences of less than a tile take four lanes each, so
+// scalar formula (1024 pairs, one a wave: 6.9 us). Sequences of less than a tile take four lanes each, so
 // that a wave has eight pairs on the way (200000 pairs of short sequences: the forward 226 us with 32 lanes each,
 // 89 us with four).
 //
@@ -525,7 +526,7 @@ __global__ __launch_bounds__(kPairThreads) void preference_pairs_kernel(Sequence
   else parts[blockIdx.x] = PairPart{all, bad};
 }
 
-// Few tokens in one workgroup: their sums, then the pairs. (Four pairs, 2620 tokens: 6.2 us, in two
+// Few tokens in one workgroup: their sums, then the pairs. (Four pairs, 2620 tokens: 6.5 us, in two
 // launches 8.5 us.)
 template <typename T>
 __global__ __launch_bounds__(kPairThreads) void preference_small_kernel(const T* __restrict__ logps,
@@ -689,7 +690,6 @@ struct Tokens {
   }
 };
 
-// A workgroup's sums; n: its tokens, or NaN where an offset is not what it has to be.
 // 1 / x of a finite x >= 1, to a rounding or two: the hardware's approximation and two steps of Newton's method
 // (the division takes twice the instructions and registers).
 __device__ __forceinline__ double reciprocal(double x) {
@@ -698,6 +698,7 @@ __device__ __forceinline__ double reciprocal(double x) {
   return __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
 }
 
+// A workgroup's sums; n: its tokens, or NaN where an offset is not what it has to be.
 struct PolicySums {
   double loss, kl, cut, n;
 };
@@ -966,8 +967,8 @@ __device__ __forceinline__ void put_policy(const PolicySums& v, T* loss, T* kl, 
 }
 
 // One pass over the tokens: losses summed, gradients written. Bound by its reads and writes (16384 x 1024
-// tokens with a mask and a reference, 285 MB: 49.8 us, 5.7 TB/s; 8.4M ragged tokens with advantages of their
-// own, 134 MB: 26.7 us, 5.0 TB/s; workgroups of 128 and 512 threads take 3 and 5 us more, longer runs of tiles by
+// tokens with a mask and a reference, 285 MB: 50.5 us, 5.6 TB/s; 8.4M ragged tokens with advantages of their
+// own, 134 MB: 26.6 us, 5.0 TB/s; workgroups of 128 and 512 threads take 3 and 5 us more, longer runs of tiles by
 // one wave 2 to 14 us). Workgroups leave their sums to policy_join_kernel: a last workgroup that sums them after a
 // device-wide fence in each cost 160 us more.
 template <typename T, int U>
@@ -1003,7 +1004,7 @@ __global__ __launch_bounds__(kPairThreads) void policy_join_kernel(const PolicyS
   if (threadIdx.x == 0) put_policy(PolicySums{v[0], v[1], v[2], v[3]}, loss, kl, cut);
 }
 
-// Few tokens in one workgroup: counted, then summed. (Eight sequences, 1616 tokens: 6.6 us, in three launches
+// Few tokens in one workgroup: counted, then summed. (Eight sequences, 1616 tokens: 6.8 us, in three launches
 // 15 us.)
 template <typename T>
 __global__ __launch_bounds__(kCountThreads) void policy_small_kernel(PolicyInputs<T> in, Sequences seq, double* weights,
@@ -1025,7 +1026,8 @@ __global__ __launch_bounds__(kCountThreads) void policy_small_kernel(PolicyInput
   if (seq.offsets != nullptr && __syncthreads_or(bad) != 0) void_gradient<kCountThreads>(in.mask, seq.total, in.grad);
 }
 
-// grad times g; a g of one leaves it as it is.
+// grad times g; a g of one leaves it as it is (1.7 us), any other costs a read and a write of it (16384 x 1024
+// tokens, 134 MB: 25.4 us, 5.3 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void policy_scale_kernel(T* __restrict__ grad, int64_t total,
                                                                 const T* __restrict__ g) {
@@ -1126,7 +1128,8 @@ hipError_t preference(const PreferenceArgs& a, void* work) {
     sums<<<dim3(static_cast<unsigned>(blocks_of(tiles_of(seq.total)))), dim3(kThreads), 0, a.stream>>>(
         logps, ref, a.mask, seq, w.first, w.last, w.whole);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // (a few lanes a sequence of few tiles)
+    // (a few lanes a sequence of few tiles, by the mean length: 19999 of 100 tokens and one of 4 million take 95 us,
+    // as many tokens spread evenly 26 us)
     const bool few = seq.total / seq.count < places;
     const int64_t each = kPairThreads / 64 * (few ? 8 : 1), want = (pairs + each - 1) / each;
     const int64_t blocks = want < kPairBlocks ? want : kPairBlocks;
@@ -1173,8 +1176,10 @@ hipError_t policy(const PolicyArgs& a, void* work) {
     const bool mean = a.reduction == TI_REDUCE_MEAN, by_sequence = a.reduction == TI_REDUCE_SEQUENCES;
     int blocks = 0;
     if (seq.total > 0 && a.mask != nullptr && (mean || by_sequence)) {
-      // masked sequences counted by as many threads as their length asks for (20000 of 1 to 600 tokens, the policy
-      // loss: by 8 threads each 35.7 us, by 64 41.7 us; 8000 of 1 to 2000: 49.3 and 45.2 us); else the places in turn
+      // masked sequences counted by as many threads as their mean length asks for (20000 of 1 to 600 tokens, the
+      // policy loss: by 8 threads each 35.7 us, by 64 41.7 us; 8000 of 1 to 2000: 49.3 and 45.2 us), which a sequence
+      // far longer than the mean waits for (20000 of 200 tokens and one of 131072: 321 us, as many tokens spread
+      // evenly 29 us; 19999 of 100 and one of 4 million: 9.0 ms and 38 us); else the places in turn
       const int64_t length = seq.total / seq.count;
       const int lanes = mean ? 64 : (length >= 32768 ? kCountThreads : (length >= 512 ? 64 : 8));
       const int64_t want = mean ? (seq.total + 16383) / 16384 : (seq.count + kCountThreads / lanes - 1) / (kCountThreads / lanes);

@@ -14,7 +14,8 @@ pads), whatever their values. ``token_logprobs`` gives the log-probabilities.
   divergence from the reference. Advantages of a group of samples may be their soft ranks.
 
 The tokens' sums, the losses and the gradients run in HIP kernels (``ti_preference``, ``ti_policy``);
-sums are float64 in a fixed order. Nothing waits for the GPU: offsets on the GPU that are not what they
+sums are float64 in a fixed order, but that a policy loss's first adds the terms of four float32 tokens
+in float32. Nothing waits for the GPU: offsets on the GPU that are not what they
 have to be make the loss and the gradient of every unmasked token NaN instead of raising (of single
 losses, the pairs' whose own they are: no other can then be relied on). The reference has no counterpart.
 """
@@ -184,8 +185,12 @@ def policy_loss(
 
     plus, given ``reference_logps``, kl_coef (exp(d) - 1 - d) with d = reference_logps - logps.
     ``reduction``: "token_mean" over all tokens, "sequence_mean" (the mean over all sequences of each
-    one's mean over its tokens) or "sum"; of no tokens, 0. The gradient goes to ``logps``. float16 and
-    bfloat16 are computed in float32."""
+    one's mean over its tokens) or "sum"; of no tokens, 0. float16 and bfloat16 are computed in float32.
+
+    The gradient goes to ``logps``. Where one may be asked for, it is computed with the loss and held (a
+    value a token, not seen by saved-tensor hooks) until the backward, which multiplies it by the upstream
+    gradient in one more read and write, or leaves it where that is one: ``loss / k`` costs that pass, a
+    coefficient that is in ``advantages`` and ``kl_coef`` already does not."""
     x = _tokens(logps)
     old = _constant("old_logps", old_logps, x)
     ref = None if reference_logps is None else _constant("reference_logps", reference_logps, x)
